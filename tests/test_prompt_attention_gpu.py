@@ -11,7 +11,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tritonforge_b200 import kernels
+from tritonforge_b200 import _lib, kernels
 
 pytestmark = pytest.mark.gpu
 
@@ -219,3 +219,28 @@ def test_masked_places_beyond_whole_rounds():
     got = kernels.prompt_attention(q, k, v, cu([610]), cu([5003]))
     assert torch.isnan(got[-1]).all()
     check(got[:-1], q[:-1], k[:-1], want[:-1], [609], [5002])
+
+
+def test_a_nan_in_every_pair():
+    """12000 prompts of two tokens, a pair of tiles each, with a NaN in one channel
+    of every second token's value: each of a CTA's 81 or more pairs meets it. The
+    first tokens see their own value alone, so they return it exactly."""
+    n, h, d = 12000, 128, 64
+    q, k, v = inputs(2 * n, 2 * n, h, 1, d, torch.bfloat16)
+    v[1::2, :, 5] = float("nan")
+    got = kernels.prompt_attention(q, k, v, cu([2] * n))
+    assert torch.equal(got[0::2], v[0::2].expand(n, h, d))
+    assert torch.isnan(got[1::2, :, 5]).all()
+    keep = [c for c in range(d) if c != 5]
+    for a in range(0, n, 1000):  # the second tokens: two weights each
+        qs = q[2 * a + 1:2 * a + 2001:2].double()
+        ks, vs = (t[2 * a:2 * a + 2000].double().view(1000, 2, d) for t in (k, v))
+        p = torch.softmax(qs @ ks.transpose(1, 2) * d ** -0.5, -1)
+        e = (qs.abs() @ ks.abs().transpose(1, 2) * d ** -0.5).amax(-1, keepdim=True)
+        e = torch.expm1(2 * (d + 4) * 2.0 ** -24 * e)
+        vs = vs[..., keep]
+        want, av = p @ vs, p @ vs.abs()
+        off = (got[2 * a + 1:2 * a + 2001:2][..., keep].double() - want).abs()
+        u = U[torch.bfloat16]
+        assert (off <= u * want.abs() + (u + 2.0 ** -16 + e) * av).all()
+    assert _lib.prompt_workspaces.errors() == 0

@@ -34,9 +34,9 @@
 // unrounded values.
 // Masked values are multiplied by p = 0, so one that is not finite turns rows
 // that do not see it into NaN. A CTA that meets a non-finite output runs the
-// pair once more at its end, with such values replaced by zero in shared memory: rows
-// that do not see them come out as if they were not there, and the others are
-// computed on the CUDA cores.
+// pair once more when its slot is free again, with such values replaced by zero in
+// shared memory: rows that do not see them come out as if they were not there, and
+// the others are computed on the CUDA cores.
 //
 // 8192 tokens of 64 / 8 heads of 128: 845 us, 79% of the measured tensor rate (980
 // in a run of seconds, under the power cap); 701 queries over 9702 keys 94 us; 4099
@@ -154,8 +154,6 @@ constexpr int kThreads = 32 * (kSoftmaxWarps + 4);  // and a warpgroup of TMA, M
 constexpr int kRegsSoftmax = 208, kRegsControl = 88;
 constexpr float kRaise = 8.f;              // log2 of how far a score may pass the running maximum
 
-constexpr int kRedo = 64;                  // pairs of a CTA to be run again, at most (beyond: row by row)
-
 // What the CTA works on next: two tiles of `nt` tokens of one sequence and kv
 // head, over a range of key blocks.
 struct Item {
@@ -164,10 +162,10 @@ struct Item {
   int b0, nb[2];      // first key block, blocks of each tile from there
   int split;          // range of `splits`, or -1: all of it
   int index;          // of the pair and kv head, for `pieces`
-  int seq, pair;
+  int pair;
   int valid, clean;   // clean: non-finite values are replaced by zero
   int first_bad;      // clean: first key whose value is not finite
-  int dirty;
+  int dirty;          // met a non-finite output: to be cleaned
 };
 
 template <int D>
@@ -176,7 +174,7 @@ struct Layout {
   static constexpr int kSlots = D == 128 ? 4 : 8;        // K and V blocks in flight
   static constexpr int kRing = 2 * kTile;                // after the two Q tiles
   static constexpr int kOut = kRing + kSlots * kTile;    // a 32 x 64 piece of the output per softmax warp
-  static constexpr int kBars = kOut + 8 * 4096;          // barriers, items, the pairs to run again
+  static constexpr int kBars = kOut + 8 * 4096;          // barriers, items
   static constexpr int kBytes = kBars + 1024 + 1024;     // + alignment of the base to 1024
   // At D = 64 the lower half of S is made as soon as P's first part is written,
   // for the maximum to start on (6000 tokens, 14 / 2 heads: 130 -> 118 us). At
@@ -198,8 +196,6 @@ struct Control {
   uint64_t item_full[2], item_free[2];
   uint64_t idle;                      // every product complete
   Item item[2];
-  int redo[kRedo][2];                 // (sequence, pair x hkv + kv head)
-  int redo_count;
   int abort;
   uint32_t tmem;
 };
@@ -378,7 +374,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&ct.item_free[w], kSoftmaxWarps + 1);
     }
     mbar_init(&ct.idle, 1);
-    ct.redo_count = 0;
     ct.abort = 0;
     fence_mbarrier_init();
   }
@@ -411,15 +406,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity & 1u))) return true;
     return wait(bar, parity, 2);
   };
-  // this pair is to be run again (one lane)
-  auto note = [&](Item& item) {
-    if (atomicExch(&item.dirty, 1)) return;
-    const int at = atomicAdd(&ct.redo_count, 1);
-    if (at < kRedo) {
-      ct.redo[at][0] = item.seq;
-      ct.redo[at][1] = item.pair * a.hkv + item.kh;
-    }
-  };
 
   // (a warpgroup's warps execute the same setmaxnreg)
   if (warp >= kSoftmaxWarps) {
@@ -439,10 +425,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int items = uncut + (heads - uncut) * a.splits;
       int n_items = 0, n_q = 0, it = 0;
       bool ok = true;
-      auto emit = [&](const Span& sp, int seq, int pair, int kh, int split, int index, int clean) {
+      // into the next slot, which is free
+      auto put = [&](const Span& sp, int pair, int kh, int split, int index, int clean) {
         const int slot = n_items & 1;
-        if (n_items >= 2) ok = ok && wait(&ct.item_free[slot], (uint32_t)(n_items / 2 - 1), 1);
-        if (!ok) return;
         Item t;
         t.sp = sp;
         t.kh = kh;
@@ -466,9 +451,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         t.split = split;
         t.index = index;
-        t.seq = seq;
         t.pair = pair;
-        t.valid = seq >= 0;
+        t.valid = 1;
         t.clean = clean;
         t.first_bad = INT32_MAX;
         t.dirty = 0;
@@ -503,26 +487,49 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         ok = !*abort_flag;
       };
-      for (int id = blockIdx.x; ok && id < items;) {
-        int next = 0;
-        if (lane == 0) next = atomicAdd(a.next, 1);
-        int seq, pair;
-        const int range = id < uncut ? -1 : (id - uncut) % a.splits;
-        const int g = id < uncut ? id : uncut + (id - uncut) / a.splits;
-        pairs.find(a, g / a.hkv, seq, pair);
+      // waits for item i: true if it met a non-finite output and is to be run again
+      auto dirty = [&](int i) {
+        ok = ok && wait(&ct.item_free[i & 1], (uint32_t)(i / 2), 1);
+        return ok && __shfl_sync(0xffffffffu, *(volatile int*)&ct.item[i & 1].dirty, 0) != 0;
+      };
+      int id = blockIdx.x, next = 0;
+      for (;;) {
+        // the item that held the next slot; at the end the one in the other slot too
+        const bool more = id < items;
+        int old = n_items - 2;
+        bool again = old >= 0 && dirty(old);
+        if (!more && !again && n_items > 0) again = dirty(old = n_items - 1);
+        if (!ok || !(more || again)) break;
         Span sp;
-        if (a.S <= 32) {
-          sp = {__shfl_sync(0xffffffffu, pairs.mine.q0, seq), __shfl_sync(0xffffffffu, pairs.mine.lq, seq),
-                __shfl_sync(0xffffffffu, pairs.mine.k0, seq), __shfl_sync(0xffffffffu, pairs.mine.lk, seq)};
+        int pair, kh, range = -1, index = 0;
+        if (again) {
+          Item& was = ct.item[old & 1];
+          sp = was.sp;
+          pair = was.pair;
+          kh = was.kh;
+          __syncwarp();
+          if (lane == 0) was.dirty = 0;
         } else {
-          sp = span_of(a, seq);
+          if (lane == 0) next = atomicAdd(a.next, 1);
+          int seq;
+          range = id < uncut ? -1 : (id - uncut) % a.splits;
+          const int g = id < uncut ? id : uncut + (id - uncut) / a.splits;
+          pairs.find(a, g / a.hkv, seq, pair);
+          if (a.S <= 32) {
+            sp = {__shfl_sync(0xffffffffu, pairs.mine.q0, seq), __shfl_sync(0xffffffffu, pairs.mine.lq, seq),
+                  __shfl_sync(0xffffffffu, pairs.mine.k0, seq), __shfl_sync(0xffffffffu, pairs.mine.lk, seq)};
+          } else {
+            sp = span_of(a, seq);
+          }
+          kh = g % a.hkv;
+          index = g - uncut;
+          if (range == 0 && lane == 0) {  // for the kernel that joins the ranges
+            a.cut[2 + 2 * index] = seq;
+            a.cut[3 + 2 * index] = pair;
+          }
         }
-        if (range == 0 && lane == 0) {  // for the kernel that joins the ranges
-          a.cut[2 + 2 * (g - uncut)] = seq;
-          a.cut[3 + 2 * (g - uncut)] = pair;
-        }
-        emit(sp, seq, pair, g % a.hkv, range, g - uncut, 0);
-        id = (int)gridDim.x + __shfl_sync(0xffffffffu, next, 0);
+        put(sp, pair, kh, range, index, again);
+        if (!again) id = (int)gridDim.x + __shfl_sync(0xffffffffu, next, 0);
       }
       if (lane == 0) {
         if (blockIdx.x == 0) {
@@ -534,19 +541,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           a.next[1] = 0;
         }
       }
-      // all read: the pairs that met a non-finite output, once more
-      for (int n = n_items - 2; ok && n < n_items; ++n)
-        if (n >= 0) ok = wait(&ct.item_free[n & 1], (uint32_t)(n / 2), 1);
-      const int redo = ok ? min(*(volatile int*)&ct.redo_count, kRedo) : 0;
-      for (int i = 0; ok && i < redo; ++i)
-        emit(span_of(a, ct.redo[i][0]), ct.redo[i][0], ct.redo[i][1] / a.hkv, ct.redo[i][1] % a.hkv, -1, 0, 1);
-      if (ok) {
+      if (ok && lane == 0) {
         const int slot = n_items & 1;  // no more
-        if (n_items >= 2) ok = wait(&ct.item_free[slot], (uint32_t)(n_items / 2 - 1), 1);
-        if (ok && lane == 0) {
-          ct.item[slot].valid = 0;
-          mbar_arrive(&ct.item_full[slot]);
-        }
+        ct.item[slot].valid = 0;
+        mbar_arrive(&ct.item_full[slot]);
       }
       if (lane == 0) {
         if (*abort_flag) {  // the copies in flight land before the CTA exits
@@ -864,10 +862,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (item.clean) {
           again = __ballot_sync(0xffffffffu, real && n > *(volatile int*)&item.first_bad);
         } else {
-          const unsigned bad = __ballot_sync(0xffffffffu, real && !finite);
-          if (bad && lane == 0) note(item);
-          __syncwarp();
-          if (*(volatile int*)&ct.redo_count > kRedo) again = bad;  // perhaps not on the list
+          if (__any_sync(0xffffffffu, real && !finite) && lane == 0) *(volatile int*)&item.dirty = 1;
         }
         while (again) {
           const int src = __ffs(again) - 1;
