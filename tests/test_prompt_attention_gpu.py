@@ -244,3 +244,77 @@ def test_a_nan_in_every_pair():
         u = U[torch.bfloat16]
         assert (off <= u * want.abs() + (u + 2.0 ** -16 + e) * av).all()
     assert _lib.prompt_workspaces.errors() == 0
+
+
+def poison(v, places):
+    """v with (key, channels, value) set in every head; the channels that stay as they were."""
+    v, d = v.clone(), v.shape[2]
+    for key, channels, x in places:
+        v[key, :, channels] = x
+    bad = {c for _, channels, _ in places for c in channels}
+    return v, [c for c in range(d) if c not in bad]
+
+
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hq,hkv,d,lq,lk", [
+    (8, 2, 64, 6000, 6000), (14, 2, 64, 6000, 6000), (8, 2, 128, 3001, 6000), (64, 8, 128, 610, 6000),
+    (8, 2, 64, 16, 70000), (8, 8, 128, 40, 70000)])
+def test_values_that_are_not_finite_stay_in_their_channel(hq, hkv, d, lq, lk, dtype):
+    """Single values that are infinite or NaN, seen by nearly every query, by some and
+    by none: a query's output is the infinity, or NaN where it sees both signs or a
+    NaN, in these channels alone; all else comes out bit for bit as without them."""
+    q, k, v = inputs(lq, lk, hq, hkv, d, dtype)
+    late = lk - lq // 2 - 3
+    places = [(3, [7], NAN), (10, [9], INF), (late, [9], -INF), (lk // 2, [1], -INF), (late, [40], INF),
+              (lk - 1, [d - 1, 33], NAN), (5, [33], INF)]
+    bad, same = poison(v, places)
+    want = kernels.prompt_attention(q, k, v, cu([lq]), cu([lk]))
+    got = kernels.prompt_attention(q, k, bad, cu([lq]), cu([lk]))
+    assert torch.equal(got[..., same], want[..., same])
+    pos = torch.arange(lk - lq, lk, device="cuda")[:, None].expand(lq, hq)
+    for c in sorted(set(range(d)) - set(same)):
+        seen = {s: torch.zeros(lq, hq, dtype=torch.bool, device="cuda") for s in ("nan", "up", "down")}
+        for key, channels, x in places:
+            if c in channels:
+                seen["nan" if x != x else "up" if x > 0 else "down"] |= pos >= key
+        nan = seen["nan"] | (seen["up"] & seen["down"])
+        expect = torch.where(seen["up"], INF, torch.where(seen["down"], -INF, want[..., c].float()))
+        assert torch.equal(torch.isnan(got[..., c]), nan), c
+        assert torch.equal(got[..., c].float()[~nan], expect[~nan]), c
+    assert _lib.prompt_workspaces.errors() == 0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq,lk", [([700, 300], [700, 300]), ([9, 4], [9000, 5000])])
+def test_keys_and_queries_that_are_not_finite(lq, lk, d):
+    """NaN in a key: the whole rows that see it are NaN, also where a value is infinite; NaN in a query: its row."""
+    q, k, v = inputs(sum(lq), sum(lk), 8, 2, d, torch.bfloat16)
+    want = kernels.prompt_attention(q, k, v, cu(lq), cu(lk))
+    k[lk[0] - 5, 1, 3] = NAN  # kv head 1 (query heads 4 to 7): the first sequence's last five queries
+    v[2, 1, 6] = INF
+    q[-2, 2, 0] = NAN
+    got = kernels.prompt_attention(q, k, v, cu(lq), cu(lk))
+    nan = torch.zeros_like(got, dtype=torch.bool)
+    nan[lq[0] - 5:lq[0], 4:] = True
+    nan[-2, 2] = True
+    inf = torch.zeros_like(nan)
+    inf[max(0, 2 - lk[0] + lq[0]):lq[0], 4:, 6] = True
+    inf &= ~nan
+    assert torch.equal(torch.isnan(got), nan)
+    assert (got[inf] == INF).all()
+    assert torch.equal(got[~(nan | inf)], want[~(nan | inf)])
+
+
+def test_not_causal_values_that_are_not_finite():
+    """Every query of the sequence sees the value, no query of the other does."""
+    lens = [130, 70]
+    q, k, v = inputs(200, 200, 28, 4, 128, torch.float16)
+    want = kernels.prompt_attention(q, k, v, cu(lens), causal=False)
+    v[150, 1, 77] = NAN
+    got = kernels.prompt_attention(q, k, v, cu(lens), causal=False)
+    nan = torch.zeros_like(got, dtype=torch.bool)
+    nan[130:, 7:14, 77] = True
+    assert torch.equal(torch.isnan(got), nan) and torch.equal(got[~nan], want[~nan])

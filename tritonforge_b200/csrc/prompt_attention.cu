@@ -34,9 +34,10 @@
 // unrounded values.
 // Masked values are multiplied by p = 0, so one that is not finite turns rows
 // that do not see it into NaN. A CTA that meets a non-finite output runs the
-// pair once more when its slot is free again, with such values replaced by zero in
-// shared memory: rows that do not see them come out as if they were not there, and
-// the others are computed on the CUDA cores.
+// pair (or the range of its keys) once more when its slot is free again, with such
+// values replaced by zero in shared memory and the first key of each channel's noted:
+// rows that do not see them come out as if they were not there, and in the others
+// the channel becomes what the sum is, an infinity or NaN.
 //
 // 8192 tokens of 64 / 8 heads of 128: 845 us, 79% of the measured tensor rate (980
 // in a run of seconds, under the power cap); 701 queries over 9702 keys 94 us; 4099
@@ -92,59 +93,6 @@ __device__ __forceinline__ int keys_seen(const PromptArgs& a, const Span& sp, in
   return n < 0 ? 0 : (n > sp.lk ? sp.lk : n);
 }
 
-// One query head of one query, by a warp on the CUDA cores, over exactly the
-// keys it sees: for rows that see a value that is not finite (below).
-template <typename T, int D>
-__device__ __forceinline__ void one_row(const PromptArgs& a, const Span& sp, int i, int h) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31, kh = h / (a.hq / a.hkv);
-  const int n = keys_seen(a, sp, i);
-  const int64_t t = sp.q0 + i;
-  float qv[E], acc[E];
-  const T* qr = (const T*)a.q + t * a.q_t + (int64_t)h * a.q_h;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    qv[e] = Num<T>::to_f(qr[lane + 32 * e]) * a.scale;
-    acc[e] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  const T* kr = (const T*)a.k + (int64_t)sp.k0 * a.k_t + (int64_t)kh * a.k_h;
-  const T* vr = (const T*)a.v + (int64_t)sp.k0 * a.v_t + (int64_t)kh * a.v_h;
-  for (int j = 0; j < n; ++j, kr += a.k_t, vr += a.v_t) {
-    float x = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) x += qv[e] * Num<T>::to_f(kr[lane + 32 * e]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    const float mn = fmaxf(m, x);
-    const float c = m == mn ? 1.f : expf(m - mn), p = expf(x - mn);
-    l = l * c + p;
-    m = mn;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = acc[e] * c + p * Num<T>::to_f(vr[lane + 32 * e]);
-  }
-  T* o = (T*)a.out + t * a.o_t + (int64_t)h * a.o_h;
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[lane + 32 * e] = Num<T>::from_f(n > 0 ? acc[e] / l : 0.f);
-}
-
-// Second pass: a warp replaces the values of a V block in shared memory that
-// are not finite by zero, before the tensor cores read it, and notes the first
-// key of the sequence (key0: the block's first) that has one.
-template <typename T>
-__device__ __forceinline__ void clean_block(uint8_t* block, int D, int key0, int lk, int* first_bad) {
-  constexpr uint16_t kExp = std::is_same_v<T, __half> ? 0x7C00 : 0x7F80;
-  uint16_t* v = reinterpret_cast<uint16_t*>(block);
-  for (int e = threadIdx.x & 31; e < 128 * D; e += 32)
-    if ((v[e] & kExp) == kExp) {
-      const int key = key0 + (e / 64) % 128;  // 64 channels (128 bytes) per key and half
-      if (key < lk) atomicMin(first_bad, key);
-      v[e] = 0;
-    }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  __syncwarp();
-}
-
 constexpr int kRows = 128;                 // rows of a tile, keys of a block
 constexpr int kSoftmaxWarps = 8;           // four per tile
 constexpr int kThreads = 32 * (kSoftmaxWarps + 4);  // and a warpgroup of TMA, MMA and two idle warps
@@ -164,7 +112,6 @@ struct Item {
   int index;          // of the pair and kv head, for `pieces`
   int pair;
   int valid, clean;   // clean: non-finite values are replaced by zero
-  int first_bad;      // clean: first key whose value is not finite
   int dirty;          // met a non-finite output: to be cleaned
 };
 
@@ -175,7 +122,8 @@ struct Layout {
   static constexpr int kRing = 2 * kTile;                // after the two Q tiles
   static constexpr int kOut = kRing + kSlots * kTile;    // a 32 x 64 piece of the output per softmax warp
   static constexpr int kBars = kOut + 8 * 4096;          // barriers, items
-  static constexpr int kBytes = kBars + 1024 + 1024;     // + alignment of the base to 1024
+  static constexpr int kControl = 1536;
+  static constexpr int kBytes = kBars + kControl + 1024;  // + alignment of the base to 1024
   // At D = 64 the lower half of S is made as soon as P's first part is written,
   // for the maximum to start on (6000 tokens, 14 / 2 heads: 130 -> 118 us). At
   // D = 128 S of 64 keys takes as long as of 96 (Q's rows come from shared memory
@@ -195,10 +143,53 @@ struct Control {
   uint64_t o_full[2];                 // [tile] O complete
   uint64_t item_full[2], item_free[2];
   uint64_t idle;                      // every product complete
+  uint64_t bad_full;                  // `bad` is of the whole item
+  // of the item that is being cleaned: first key of each channel whose value is +inf or NaN, -inf or NaN
+  int bad[2][D];
   Item item[2];
   int abort;
   uint32_t tmem;
 };
+
+// Second pass: a warp replaces the values of a V block in shared memory that
+// are not finite by zero, before the tensor cores read it, and notes the first
+// key of the sequence (key0: the block's first) of each channel's.
+template <typename T, int D>
+__device__ __forceinline__ void clean_block(uint8_t* block, int key0, int lk, int (*bad)[D]) {
+  constexpr uint32_t kExp = std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u;
+  uint4* v = reinterpret_cast<uint4*>(block);
+#pragma unroll 1
+  for (int i = threadIdx.x & 31; i < kRows * D / 8; i += 32) {
+    const uint4 x = v[i];
+    uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) any |= ((w[e / 2] >> (16 * (e & 1))) & kExp) == kExp;
+    if (!any) continue;
+    // 64 channels (128 bytes, their 16-byte units swizzled) per key and half
+    const int in = (i / 8) % kRows, key = key0 + in, d0 = i / (8 * kRows) * 64 + ((i ^ in) & 7) * 8;
+#pragma unroll 1
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t h = (w[0] >> (16 * (e & 1))) & 0xffffu;
+      if ((h & kExp) == kExp) {
+        w[0] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
+        const bool nan = (h & 0x7fffu) != kExp;
+        if (key < lk && (nan || h == kExp)) atomicMin(&bad[0][d0 + e], key);
+        if (key < lk && (nan || h != kExp)) atomicMin(&bad[1][d0 + e], key);
+      }
+      if (e & 1) {  // the next word to the front
+        const uint32_t done = w[0];
+        w[0] = w[1];
+        w[1] = w[2];
+        w[2] = w[3];
+        w[3] = done;
+      }
+    }
+    v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+}
 
 // 32 columns of this warp's 32 lanes (one lane per thread): the load, and the
 // wait after which the registers may be used.
@@ -351,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   Control<D>& ct = *reinterpret_cast<Control<D>*>(smem + L::kBars);
-  static_assert(sizeof(Control<D>) <= 1024, "control block");
+  static_assert(sizeof(Control<D>) <= L::kControl, "control block");
   volatile int* abort_flag = &ct.abort;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -374,6 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&ct.item_free[w], kSoftmaxWarps + 1);
     }
     mbar_init(&ct.idle, 1);
+    mbar_init(&ct.bad_full, 1);
     ct.abort = 0;
     fence_mbarrier_init();
   }
@@ -454,7 +446,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         t.pair = pair;
         t.valid = 1;
         t.clean = clean;
-        t.first_bad = INT32_MAX;
         t.dirty = 0;
         if (lane == 0) {
           ct.item[slot] = t;
@@ -501,12 +492,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!more && !again && n_items > 0) again = dirty(old = n_items - 1);
         if (!ok || !(more || again)) break;
         Span sp;
-        int pair, kh, range = -1, index = 0;
+        int pair, kh, range, index;
         if (again) {
           Item& was = ct.item[old & 1];
           sp = was.sp;
           pair = was.pair;
           kh = was.kh;
+          range = was.split;
+          index = was.index;
           __syncwarp();
           if (lane == 0) was.dirty = 0;
         } else {
@@ -595,7 +588,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int k = k0; k < k1; ++k)
               mma_ts(leader, tm + 256 + tile * D, pa + k * 8, va + k * (2048 >> 4), a.idesc_o, (k > k0 || !first) ? 1u : 0u);
           };
-          ok = ready(&ct.q_full, (uint32_t)n_q) && ready(&ct.full[slot], slot_phase);
+          if (clean) {  // what `bad` holds is read until the item before is done
+            ok = wait(&ct.item_free[(n_items - 1) & 1], (uint32_t)((n_items - 1) / 2), 2);
+            for (int e = lane; e < 2 * D; e += 32) (&ct.bad[0][0])[e] = INT32_MAX;
+            __syncwarp();
+          }
+          ok = ok && ready(&ct.q_full, (uint32_t)n_q) && ready(&ct.full[slot], slot_phase);
           ++n_q;
           if (ok) {
             tc_fence_after();
@@ -621,8 +619,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               ok = ready(&ct.full[slot], slot_phase);
               next_slot();
             }
-            if (ok && clean)
-              clean_block<T>(smem + L::kRing + v_slot * L::kTile, D, (item.b0 + j) * kRows, item.sp.lk, &item.first_bad);
+            if (ok && clean) {
+              clean_block<T, D>(smem + L::kRing + v_slot * L::kTile, (item.b0 + j) * kRows, item.sp.lk, ct.bad);
+              if (j + 1 == nb && lane == 0) mbar_arrive(&ct.bad_full);
+            }
 #pragma unroll
             for (int tile = 0; tile < 2; ++tile) {
               const int n = tile ? n1 : n0;
@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lanes + tile * 128, o_addr = tmem + lanes + 256 + tile * D;
     const float c = a.scale * 1.4426950408889634f;
-    uint32_t done = 0, n_o = 0;  // blocks and O products so far
+    uint32_t done = 0, n_o = 0, n_clean = 0;  // blocks, O products and cleaned items so far
     bool ok = true;
     for (int n_items = 0; ok; ++n_items) {
       ok = wait(&ct.item_full[n_items & 1], (uint32_t)(n_items / 2), 2);
@@ -780,7 +780,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         ++n_o;
       }
+      if (item.clean) {
+        ok = wait(&ct.bad_full, n_clean, 2);
+        if (!ok) break;
+        ++n_clean;
+      }
       tc_fence_after();
+      // of a cleaned item: what channel d of this row's sum is, where the row sees a value that is not finite
+      auto patch = [&](auto&& store) {
+        for (int d = 0; d < D; ++d) {
+          const bool up = n > ct.bad[0][d], down = n > ct.bad[1][d];
+          if (up || down) store(d, up && down ? NAN : up ? INFINITY : -INFINITY);
+        }
+      };
       bool finite = true;
       if (item.split < 0) {
         // Through shared memory, 64 channels at a time: a warp's stores then cover
@@ -834,6 +846,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         unpair(check2[1], c2, c3);
         const float check = (c0 + c1) + (c2 + c3);
         finite = check == check;
+        if (item.clean && real)
+          patch([&](int d, float x) { ((T*)a.out)[mine + d] = Num<T>::from_f(l > 0.f ? x : NAN); });
       } else {
         float* piece = a.pieces + (((int64_t)item.index * a.splits + item.split) * 2 + tile) * L::kPiece;
 #pragma unroll
@@ -845,6 +859,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = 0u;
           }
+          float check = 0.f;  // NaN when a sum is not finite
+#pragma unroll
+          for (int e = 0; e < 16; ++e) check = fmaf(__uint_as_float(o[e]), 0.f, check);
+          finite = finite && check == check;
           if (real)
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
@@ -855,21 +873,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (real) {
           __stcg(piece + D * kRows + row, m);
           __stcg(piece + (D + 1) * kRows + row, l);
+          if (item.clean) patch([&](int d, float x) { __stcg(piece + (d / 4 * kRows + row) * 4 + d % 4, x); });
         }
       }
-      if (item.split < 0) {
-        unsigned again = 0;  // rows to compute on the CUDA cores
-        if (item.clean) {
-          again = __ballot_sync(0xffffffffu, real && n > *(volatile int*)&item.first_bad);
-        } else {
-          if (__any_sync(0xffffffffu, real && !finite) && lane == 0) *(volatile int*)&item.dirty = 1;
-        }
-        while (again) {
-          const int src = __ffs(again) - 1;
-          again &= again - 1;
-          one_row<T, D>(a, sp, __shfl_sync(0xffffffffu, i, src), __shfl_sync(0xffffffffu, h, src));
-        }
-      }
+      if (!item.clean && __any_sync(0xffffffffu, real && !finite) && lane == 0) *(volatile int*)&item.dirty = 1;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&ct.item_free[n_items & 1]);
@@ -890,7 +897,6 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) prompt_join_kernel(const PromptArgs a) {
   constexpr int64_t kStep = 2 * Layout<D>::kPiece;
   __shared__ float weight[kMaxSplits][kRows];
-  __shared__ int dirty;
   pdl_trigger();
   pdl_wait();
   const int index = (int)(blockIdx.x >> 1), tile = (int)(blockIdx.x & 1);
@@ -901,7 +907,6 @@ __global__ void __launch_bounds__(kJoinThreads) prompt_join_kernel(const PromptA
   if (rows <= 0) return;
   const float* first = a.pieces + ((int64_t)index * a.splits * 2 + tile) * Layout<D>::kPiece;
   const float c = a.scale * 1.4426950408889634f;
-  if (threadIdx.x == 0) dirty = 0;
   if ((int)threadIdx.x < rows) {
     const int r = threadIdx.x;
     const float* ms = first + D * kRows + r;
@@ -921,7 +926,6 @@ __global__ void __launch_bounds__(kJoinThreads) prompt_join_kernel(const PromptA
     for (int k = 0; k < a.splits; ++k) weight[k][r] *= inv;
   }
   __syncthreads();
-  bool finite = true;
   for (int u = threadIdx.x; u < rows * (D / 16); u += kJoinThreads) {
     const int r = u % rows, col = u / rows;
     float4 x[4];
@@ -943,8 +947,6 @@ __global__ void __launch_bounds__(kJoinThreads) prompt_join_kernel(const PromptA
     uint32_t w[8];
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
-      const float check = fmaf(x[y].x, 0.f, fmaf(x[y].y, 0.f, fmaf(x[y].z, 0.f, x[y].w * 0.f)));  // NaN if one is not finite
-      finite = finite && check == check;
       w[2 * y] = pack2<T>(x[y].x, x[y].y);
       w[2 * y + 1] = pack2<T>(x[y].z, x[y].w);
     }
@@ -953,11 +955,6 @@ __global__ void __launch_bounds__(kJoinThreads) prompt_join_kernel(const PromptA
     o[0] = make_uint4(w[0], w[1], w[2], w[3]);
     o[1] = make_uint4(w[4], w[5], w[6], w[7]);
   }
-  if (!finite) dirty = 1;
-  __syncthreads();
-  if (dirty)  // masked values that are not finite, or rows that see one: every row over exactly its keys
-    for (int r = threadIdx.x >> 5; r < rows; r += kJoinThreads / 32)
-      one_row<T, D>(a, sp, i0 + r / G, kh * G + r % G);
 }
 
 constexpr size_t kFixedBytes = 8192;  // error word, counters, the table of pairs that were cut
