@@ -717,7 +717,7 @@ class QwenDecoder:
                 raise RuntimeError(f"{what} needs K-major projections (QwenDecoder(..., colmajor=False))")
 
     @torch.no_grad()
-    def prefill_packed(self, prompts: list[torch.Tensor]) -> torch.Tensor:
+    def prefill_packed(self, prompts: list[torch.Tensor], steps: int = 0) -> torch.Tensor:
         """Run one prompt per sequence (1-D token tensors, their lengths free),
         packed into one batch of rows, and set each sequence's first generated
         token and position (kv_bits=4). Every projection is one GEMM over all
@@ -728,7 +728,11 @@ class QwenDecoder:
         Sequences that hold tokens already are continued (the next turn of a
         conversation, a long prompt in pieces): their new tokens follow at
         positions pos[b] on, and attend over the cached positions, read back from
-        4 bits (kv4_read), their own included. `reset` starts over."""
+        4 bits (kv4_read), their own included. `reset` starts over.
+
+        Prompts that would end past the cache are refused, as are prompts that
+        leave no room for `steps` decode steps after them (a step past the cache
+        writes nothing and attends to nothing)."""
         if self.kv4 is None:
             raise RuntimeError("prefill_packed needs the 4-bit cache (QwenDecoder(..., kv_bits=4))")
         self._needs_k_major("prefill_packed")
@@ -739,8 +743,9 @@ class QwenDecoder:
         lens = [p.numel() for p in prompts]
         start = self.pos.tolist()
         ends = [a + n for a, n in zip(start, lens)]
-        if max(ends) >= self.T:
-            raise ValueError(f"prompts end at position {max(ends)}, past max_len {self.T}")
+        if max(ends) + max(steps, 1) > self.T:
+            raise ValueError(f"prompts end at position {max(ends)}" + (f", {steps} steps" if steps > 1 else "")
+                             + f": past max_len {self.T}")
         toks = torch.cat([p.reshape(-1) for p in prompts]).to(dev, torch.long)
         n, again = toks.numel(), any(start)
 
@@ -807,11 +812,18 @@ class QwenDecoder:
                         use_graph: bool = True) -> dict[str, torch.Tensor]:
         """Greedy decode of prompts of different lengths (kv_bits=4): a dict of
         tokens [B, new_tokens], their logprobs and entropies, and, for top > 0,
-        the top_ids and top_logprobs [B, new_tokens, top] of each step."""
+        the top_ids and top_logprobs [B, new_tokens, top] of each step. The
+        prompts and the new_tokens - 1 tokens that are fed back have to fit the
+        cache."""
+        if new_tokens < 1:
+            raise ValueError(f"new_tokens must be at least 1, got {new_tokens}")
         out: dict[str, list[torch.Tensor]] = {k: [] for k in ("tokens", "logprobs", "entropies", "top_logprobs",
                                                               "top_ids")}
         for i in range(new_tokens):
-            toks = self.prefill_packed(prompts) if i == 0 else (self.replay() if use_graph else self.step()).clone()
+            if i == 0:
+                toks = self.prefill_packed(prompts, steps=new_tokens - 1)
+            else:
+                toks = (self.replay() if use_graph else self.step()).clone()
             for k, t in zip(out, (toks, *self.logprobs(top))):
                 out[k].append(t)
         if not top:
