@@ -377,6 +377,7 @@ class QwenDecoder:
         self.tokens = torch.zeros(B, dtype=torch.long, device=dev)
         # [position, length = position + 1] of the batch; with the 4-bit cache each sequence's position
         self.pos = torch.zeros(B if kv_bits == 4 else 2, dtype=torch.int32, device=dev)
+        self._unfed = False  # generate_packed returned self.tokens, which the cache does not hold yet
         self.buf = {
             "x": torch.empty(B, self.H, dtype=dt, device=dev),
             "normed": torch.empty(B, self.H, dtype=dt, device=dev),
@@ -728,7 +729,11 @@ class QwenDecoder:
         Sequences that hold tokens already are continued (the next turn of a
         conversation, a long prompt in pieces): their new tokens follow at
         positions pos[b] on, and attend over the cached positions, read back from
-        4 bits (kv4_read), their own included. `reset` starts over.
+        4 bits (kv4_read), their own included. After generate_packed the last
+        token that it returned, which no step was fed, goes before the new ones.
+        After prefill_packed and steps called one by one the tokens chosen last are
+        not put in: a continuation that is to hold them begins with them. `reset`
+        starts over.
 
         Prompts that would end past the cache are refused, as are prompts that
         leave no room for `steps` decode steps after them (a step past the cache
@@ -740,6 +745,8 @@ class QwenDecoder:
             raise ValueError(f"prefill_packed takes {self.B} non-empty 1-D prompts")
         dev, dt, H, D = self.dev, self.embed.dtype, self.H, self.D
         hq, hkv = self.Hq * D, self.Hkv * D
+        if self._unfed:
+            prompts = [torch.cat([t, p.to(dev, torch.long)]) for t, p in zip(self.tokens.split(1), prompts)]
         lens = [p.numel() for p in prompts]
         start = self.pos.tolist()
         ends = [a + n for a, n in zip(start, lens)]
@@ -792,11 +799,13 @@ class QwenDecoder:
         # the head advances the positions by one: to the first generated tokens'
         self.pos.copy_(torch.tensor(ends, dtype=torch.int32) - 1)
         self._head(normed[cu[1:].long() - 1].contiguous())
+        self._unfed = False
         return self.tokens.clone()
 
     def reset(self) -> None:
         """Forget every sequence: the next prompts start at position 0."""
         self.pos.zero_()
+        self._unfed = False
 
     @torch.no_grad()
     def logprobs(self, top: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -814,7 +823,8 @@ class QwenDecoder:
         tokens [B, new_tokens], their logprobs and entropies, and, for top > 0,
         the top_ids and top_logprobs [B, new_tokens, top] of each step. The
         prompts and the new_tokens - 1 tokens that are fed back have to fit the
-        cache."""
+        cache. Sequences that hold tokens are continued (prefill_packed): called
+        again, it takes the next turn of each conversation."""
         if new_tokens < 1:
             raise ValueError(f"new_tokens must be at least 1, got {new_tokens}")
         out: dict[str, list[torch.Tensor]] = {k: [] for k in ("tokens", "logprobs", "entropies", "top_logprobs",
@@ -822,6 +832,7 @@ class QwenDecoder:
         for i in range(new_tokens):
             if i == 0:
                 toks = self.prefill_packed(prompts, steps=new_tokens - 1)
+                self._unfed = True
             else:
                 toks = (self.replay() if use_graph else self.step()).clone()
             for k, t in zip(out, (toks, *self.logprobs(top))):
@@ -953,6 +964,7 @@ class QwenDecoder:
                 kernels.kv4_write(kv.normal_(generator=g), torch.empty_like(kv).normal_(generator=g), cache, cu)
             self.tokens.copy_(torch.randint(0, self.embed.shape[0], (self.B,), generator=g, device=self.dev))
             self.pos.fill_(length)
+            self._unfed = False
             return
         for li in range(len(self.layers)):
             self.k_cache[li, :, :, :length].normal_(generator=g)
