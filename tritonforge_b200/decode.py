@@ -712,8 +712,8 @@ class QwenDecoder:
         if self.kv4 is not None:
             raise RuntimeError(f"{what} fills the 16-bit cache; with kv_bits=4 use prefill_packed")
 
-    def _needs_k_major(self, what: str) -> None:
-        for L in self.layers:
+    def _needs_k_major(self, what: str, layers: list) -> None:
+        for L in layers:
             if not all(isinstance(L[n], QuantLinear) for n in ("qkv", "o", "gu", "down")):
                 raise RuntimeError(f"{what} needs K-major projections (QwenDecoder(..., colmajor=False))")
 
@@ -725,6 +725,8 @@ class QwenDecoder:
         rows; q and k are rotated in place and the keys and values quantised into
         the cache by one kernel (rope_kv4_write), and attention over the packed
         prompts reads q, k, v where the projection left them (prompt_attention).
+        The projections are the K-major ones that the weights hold, whatever
+        layout the steps use; weights converted in place (to_colmajor) hold none.
 
         Sequences that hold tokens already are continued (the next turn of a
         conversation, a long prompt in pieces): their new tokens follow at
@@ -740,7 +742,8 @@ class QwenDecoder:
         writes nothing and attends to nothing)."""
         if self.kv4 is None:
             raise RuntimeError("prefill_packed needs the 4-bit cache (QwenDecoder(..., kv_bits=4))")
-        self._needs_k_major("prefill_packed")
+        layers = self.w.layers  # K-major, also where the steps run on column-major copies
+        self._needs_k_major("prefill_packed", layers)
         if len(prompts) != self.B or any(p.ndim != 1 or p.numel() < 1 for p in prompts):
             raise ValueError(f"prefill_packed takes {self.B} non-empty 1-D prompts")
         dev, dt, H, D = self.dev, self.embed.dtype, self.H, self.D
@@ -782,9 +785,9 @@ class QwenDecoder:
         _lib.check(self._lib.tf_embed_gather(
             self.embed.data_ptr(), self.embed.stride(0), toks.data_ptr(), x.data_ptr(), H, res.data_ptr(), H,
             self.embed.shape[0], H, n, _lib.dtype_code(dt), _lib.stream_ptr(dev)), "embed_gather")
-        kernels.rmsnorm(x, self.layers[0]["in_norm"], self.eps, out=normed)
-        nl = len(self.layers)
-        for li, L in enumerate(self.layers):
+        kernels.rmsnorm(x, layers[0]["in_norm"], self.eps, out=normed)
+        nl = len(layers)
+        for li, L in enumerate(layers):
             self._lin(normed, L["qkv"], qkv)
             kernels.rope_kv4_write(qkv, self.Hq, self.cos, self.sin, self.kv4[li], cu, self.pos)
             if again:
@@ -793,7 +796,7 @@ class QwenDecoder:
             row_parallel(attn, L["o"], L["post_norm"], res, res_next)
             res, res_next = res_next, res
             self._gate_up(normed, L["gu"], act)
-            nxt = self.layers[li + 1]["in_norm"] if li + 1 < nl else self.final_norm
+            nxt = layers[li + 1]["in_norm"] if li + 1 < nl else self.final_norm
             row_parallel(act, L["down"], nxt, res, res_next)
             res, res_next = res_next, res
         # the head advances the positions by one: to the first generated tokens'
@@ -895,7 +898,7 @@ class QwenDecoder:
         t0 = prompt.shape[1]
         if t0 < 1 or t0 >= self.T:
             raise ValueError(f"prompt length {t0} does not fit max_len {self.T}")
-        self._needs_k_major("prefill_tokens")
+        self._needs_k_major("prefill_tokens", self.layers)
         prompt = prompt.to(self.dev, torch.long)
         dt, dev, H, D = self.embed.dtype, self.dev, self.H, self.D
         hq, hkv = self.Hq * D, self.Hkv * D
