@@ -221,3 +221,43 @@ def test_near_tie_check():
     assert logits_close(bumped, base)[0]
     bumped[0, 1] += 0.12 * rms  # beyond one bf16 ulp of any value here plus the 6e-2 x RMS bound
     assert not logits_close(bumped, base)[0]
+
+
+def _gather_worker(rank, world, port, q):
+    try:
+        _init(rank, world, port)
+        from tritonforge_b200.tp import gather_vocab
+
+        ok = True
+        for b, vocab in ((1, 7), (3, 1001), (2, 6)):
+            for dtype in (torch.bfloat16, torch.float32):
+                logits = torch.randn(b, vocab, generator=torch.Generator().manual_seed(vocab)).to(dtype)
+                v0, v1 = split_even(vocab, world, rank)
+                got = gather_vocab(logits[:, v0:v1], vocab)
+                ok &= got.dtype == dtype and torch.equal(got, logits)
+        try:
+            gather_vocab(torch.zeros(2, 5), 1001)
+            ok = False
+        except ValueError:
+            pass
+        q.put((rank, ok, None))
+        dist.barrier()
+        dist.destroy_process_group()
+    except Exception as e:  # pragma: no cover - reported to the parent
+        q.put((rank, False, repr(e)))
+
+
+@pytest.mark.parametrize("world", [2, 3])
+def test_gather_vocab_gloo(world):
+    """The ranks' slices of the logits, even and uneven, side by side again on every rank."""
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    port = _free_port()
+    procs = [ctx.Process(target=_gather_worker, args=(r, world, port, q)) for r in range(world)]
+    for p in procs:
+        p.start()
+    results = [q.get(timeout=120) for _ in range(world)]
+    for p in procs:
+        p.join(timeout=60)
+    for rank, ok, info in results:
+        assert ok, (rank, info)

@@ -814,10 +814,14 @@ class QwenDecoder:
     def logprobs(self, top: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
         """(logprob [B], entropy [B], top_logprobs [B, top], top_ids [B, top]) of
         the tokens chosen last, from the logits that the head left
-        (kernels.token_logprobs). Not for a vocabulary split over ranks."""
+        (kernels.token_logprobs). With the vocabulary split over ranks they are
+        gathered first: every rank calls it and gets the same."""
+        logits = self.buf["logits"]
         if self.vocab_parallel:
-            raise RuntimeError("logprobs needs the whole vocabulary (vocab_parallel=False)")
-        return kernels.token_logprobs(self.buf["logits"], self.tokens, top)
+            from .tp import gather_vocab
+
+            logits = gather_vocab(logits, self.vocab, self.group)
+        return kernels.token_logprobs(logits, self.tokens, top)
 
     @torch.no_grad()
     def generate_packed(self, prompts: list[torch.Tensor], new_tokens: int, top: int = 0,

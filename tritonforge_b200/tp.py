@@ -123,6 +123,24 @@ def best_of_ranks(all_best: torch.Tensor) -> torch.Tensor:
     return torch.gather(all_best[:, :, 1], 0, win.unsqueeze(0)).squeeze(0)
 
 
+def gather_vocab(part: torch.Tensor, vocab: int, group=None) -> torch.Tensor:
+    """Logits [B, vocab] from every rank's slice `part` [B, V_local] (split_even
+    of the vocabulary, in rank order): a collective, every rank of the group
+    calls it. Slices travel padded to the widest."""
+    import torch.distributed as dist
+
+    world, rank = dist.get_world_size(group), dist.get_rank(group)
+    spans = [split_even(vocab, world, r) for r in range(world)]
+    b, n = part.shape
+    if n != spans[rank][1] - spans[rank][0]:
+        raise ValueError(f"rank {rank} of {world} holds {n} of {vocab} logits")
+    width = spans[0][1] - spans[0][0]
+    mine = part if n == width else torch.nn.functional.pad(part, (0, width - n))
+    every = torch.empty(world * b, width, dtype=part.dtype, device=part.device)
+    dist.all_gather_into_tensor(every, mine.contiguous(), group=group)
+    return torch.cat([every[r * b:(r + 1) * b, :v1 - v0] for r, (v0, v1) in enumerate(spans)], dim=1)
+
+
 def interleave_gate_up(gate: torch.Tensor, up: torch.Tensor, block: int = 64) -> torch.Tensor:
     """Columns of gate [R, I] and up [R, I] interleaved per `block` columns:
     [gate 0:64 | up 0:64 | gate 64:128 | up 64:128 | ...] (the layout the fused
