@@ -359,3 +359,44 @@ def test_codes_at_and_around_halves(dtype):
         c, p = quantize(y, 64)
         assert same_bits(cache[side][0, 0, :n], c[:, 0])
         assert same_bits(cache[side + 1][0, 0, :n], p[:, 0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_one_token_or_one_head_of_odd_strides(dtype):
+    """An axis of one element may have any stride, as in a row cut from a wider one."""
+    h, hq, d, g = 2, 4, 64, 64
+    k, v = tokens(1, h, d, dtype)
+
+    def one(x):  # heads 72 apart, the token 147 from a next one
+        buf = torch.zeros(h * (d + 8), device="cuda", dtype=dtype)
+        return torch.as_strided(buf, (1, h, d), (h * (d + 8) + 3, d + 8, 1)).copy_(x)
+
+    want, got = (KV4Cache.empty(1, h, 32, d, g, dtype) for _ in range(2))
+    kernels.kv4_write(k, v, want, cu([1]), i32(5))
+    kernels.kv4_write(one(k), one(v), got, cu([1]), i32(5))
+    assert all(same_bits(a, b) for a, b in zip(got, want))
+    for x, y in zip(kernels.kv4_read(got, cu([1]), 1, i32(5), out=(one(k), one(v))),
+                    kernels.kv4_read(got, cu([1]), 1, i32(5))):
+        assert torch.equal(x, y)
+    # the projection row of one token
+    width = (hq + 2 * h) * d
+    row = torch.randn(1, width, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).to(dtype)
+    whole, qkv = row.clone(), torch.as_strided(row, (1, width), (width + 3, 1))
+    ang = torch.rand(32, d // 2, device="cuda", generator=torch.Generator("cuda").manual_seed(2)) * 6
+    cos, sin = (torch.cat([f(ang), f(ang)], -1).to(dtype) for f in (torch.cos, torch.sin))
+    a = kernels.kv4_decode_attention_rope(qkv, hq, cos, sin, got, i32(6))
+    b = kernels.kv4_decode_attention_rope(whole, hq, cos, sin, want, i32(6))
+    assert torch.equal(a, b) and all(same_bits(x, y) for x, y in zip(got, want))
+    kernels.rope_kv4_write(qkv, hq, cos, sin, got, cu([1]), i32(7))
+    kernels.rope_kv4_write(whole, hq, cos, sin, want, cu([1]), i32(7))
+    assert torch.equal(qkv, whole) and all(same_bits(x, y) for x, y in zip(got, want))
+    # several tokens of one head
+    k1, v1 = tokens(5, 1, d, dtype)
+
+    def many(x):
+        return torch.as_strided(torch.zeros(5 * 72, device="cuda", dtype=dtype), x.shape, (72, 3, 1)).copy_(x)
+
+    want, got = (KV4Cache.empty(1, 1, 16, d, g, dtype) for _ in range(2))
+    kernels.kv4_write(k1, v1, want, cu([5]))
+    kernels.kv4_write(many(k1), many(v1), got, cu([5]))
+    assert all(same_bits(x, y) for x, y in zip(got, want))

@@ -153,10 +153,13 @@ int check_packed(const char* what, int64_t T, int S, const int* cu) {
   return TF_OK;
 }
 
-int check_rows(const char* what, const void* k, const void* v, int64_t k_t, int64_t k_h, int64_t v_t, int64_t v_h) {
+// (the stride of an axis of one element counts for nothing)
+int check_rows(const char* what, const void* k, const void* v, int64_t k_t, int64_t k_h, int64_t v_t, int64_t v_h,
+               int64_t T, int hkv) {
   if (!k || !v) return fail(TF_ERR_BAD_ARG, "%s: null pointer", what);
-  if (k_t < 0 || k_h < 0 || v_t < 0 || v_h < 0 || k_t % 8 || k_h % 8 || v_t % 8 || v_h % 8 || !aligned(k, 16) ||
-      !aligned(v, 16))
+  const bool tokens = T > 1 && (k_t < 0 || v_t < 0 || k_t % 8 || v_t % 8);
+  const bool heads = hkv > 1 && (k_h < 0 || v_h < 0 || k_h % 8 || v_h % 8);
+  if (tokens || heads || !aligned(k, 16) || !aligned(v, 16))
     return fail(TF_ERR_UNALIGNED, "%s: rows must be 16-byte aligned", what);
   return TF_OK;
 }
@@ -184,7 +187,7 @@ extern "C" int tf_kv4_write(const void* k, int64_t k_stride_t, int64_t k_stride_
   int rc = kv4_check("kv4_write", c, B, hkv, head_dim, group, t_max, dtype);
   if (rc == TF_OK) rc = check_packed("kv4_write", T, S, cu);
   if (rc != TF_OK || T == 0) return rc;
-  rc = check_rows("kv4_write", k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h);
+  rc = check_rows("kv4_write", k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, T, hkv);
   if (rc != TF_OK) return rc;
   const Kv4Rows a{c, cu, start, slots, T, B, t_max, S, hkv};
   return kv4_dispatch(dtype, head_dim, group, [&](auto type, auto d, auto g) {
@@ -233,7 +236,7 @@ extern "C" int tf_kv4_read(const uint8_t* k_codes, const void* k_params, const u
   int rc = kv4_check("kv4_read", c, B, hkv, head_dim, group, t_max, dtype);
   if (rc == TF_OK) rc = check_packed("kv4_read", T, S, cu);
   if (rc != TF_OK || T == 0) return rc;
-  rc = check_rows("kv4_read", k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h);
+  rc = check_rows("kv4_read", k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, T, hkv);
   if (rc != TF_OK) return rc;
   const Kv4Rows a{c, cu, start, slots, T, B, t_max, S, hkv};
   return kv4_dispatch(dtype, head_dim, group, [&](auto type, auto d, auto g) {

@@ -89,7 +89,8 @@ def _side(t: torch.Tensor, h: int, d: int, dtype: torch.dtype, name: str) -> int
 
 
 def _rope_rows(qkv: torch.Tensor, q_heads: int, cos: torch.Tensor, sin: torch.Tensor, cache: KV4Cache, h: int, d: int,
-               t_max: int) -> None:
+               t_max: int) -> int:
+    """The row stride of projection rows that fit the cache and the tables."""
     width = (q_heads + 2 * h) * d
     if qkv.ndim != 2 or qkv.shape[1] != width or qkv.stride(1) != 1 or qkv.dtype != cache.k_params.dtype:
         raise ValueError(f"qkv must be rows of {width} {cache.k_params.dtype}, got {tuple(qkv.shape)} {qkv.dtype}")
@@ -98,6 +99,7 @@ def _rope_rows(qkv: torch.Tensor, q_heads: int, cos: torch.Tensor, sin: torch.Te
     for name, t in (("cos", cos), ("sin", sin)):
         if t.ndim != 2 or t.shape[0] < t_max or t.shape[1] != d or t.dtype != qkv.dtype or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous [>= {t_max}, {d}] of {qkv.dtype}, got {tuple(t.shape)}")
+    return qkv.stride(0) if qkv.shape[0] > 1 else width
 
 
 def kv4_write(k: torch.Tensor, v: torch.Tensor, cache: KV4Cache, cu_seqlens: torch.Tensor,
@@ -129,10 +131,10 @@ def rope_kv4_write(qkv: torch.Tensor, q_heads: int, cos: torch.Tensor, sin: torc
     kv4_write places them. Tokens outside the cache are neither rotated nor written."""
     b, h, d, g, t_max, dt = cache.layout()
     S = _offsets(cu_seqlens)
-    _rope_rows(qkv, q_heads, cos, sin, cache, h, d, t_max)
+    ld = _rope_rows(qkv, q_heads, cos, sin, cache, h, d, t_max)
     dev = _lib.require_cuda(qkv, cos, sin, *cache, cu_seqlens, start, slots)
     rc = _lib.load().tf_rope_kv4_write(
-        qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]), cos.data_ptr(), sin.data_ptr(), *cache.pointers(),
+        qkv.data_ptr(), ld, cos.data_ptr(), sin.data_ptr(), *cache.pointers(),
         cu_seqlens.data_ptr(), _index(start, S, "start"), _index(slots, S, "slots"), S, qkv.shape[0], b, q_heads, h, d,
         g, t_max, dt, _lib.stream_ptr(dev))
     _lib.check(rc, "rope_kv4_write")
@@ -207,7 +209,7 @@ def kv4_decode_attention_rope(qkv: torch.Tensor, q_heads: int, cos: torch.Tensor
     rope_kv4_write followed by kv4_decode_attention; qkv is only read. A sequence
     whose position lies outside the cache writes nothing and gets zeros."""
     b, h, d, g, t_max, dt = cache.layout()
-    _rope_rows(qkv, q_heads, cos, sin, cache, h, d, t_max)
+    ld = _rope_rows(qkv, q_heads, cos, sin, cache, h, d, t_max)
     if qkv.shape[0] != b:
         raise ValueError(f"{qkv.shape[0]} rows for a cache of {b} sequences")
     if q_heads < 1 or q_heads % h:
@@ -222,7 +224,7 @@ def kv4_decode_attention_rope(qkv: torch.Tensor, q_heads: int, cos: torch.Tensor
     lib = _lib.load()
     ws = _lib.kv4_workspaces.get(dev, lib.tf_kv4_attention_workspace_bytes())
     rc = lib.tf_kv4_decode_attention_rope(
-        qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]), cos.data_ptr(), sin.data_ptr(), *cache.pointers(),
+        qkv.data_ptr(), ld, cos.data_ptr(), sin.data_ptr(), *cache.pointers(),
         _index(pos, b, "pos"), out.data_ptr(), b, q_heads, h, d, g, t_max, d ** -0.5 if scale is None else scale, dt,
         ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev))
     _lib.check(rc, "kv4_decode_attention_rope")
