@@ -374,7 +374,8 @@ int tf_best_of_ranks(const float* all_best, int64_t* tokens, int32_t world, int6
  * tf_prompt_attention: out[i, h] = softmax_j(scale q_i . k_j) v_j over packed
  * sequences: sequence s owns queries cu_q[s] .. cu_q[s+1]-1 of q [Tq, hq, D]
  * and keys cu_k[s] .. cu_k[s+1]-1 of k, v [Tk, hkv, D] (device int32 offsets,
- * S + 1 each, cu[0] = 0, cu[S] = Tq / Tk). A sequence's queries are the last
+ * S + 1 each, non-decreasing, inside 0..Tq / 0..Tk; out rows of queries in no
+ * sequence are left as they are). A sequence's queries are the last
  * of its positions; causal queries see the keys up to their own position, and
  * a query that sees none gives zeros. Strides are of tokens and heads, in
  * elements, multiples of 8 and at least D; channels contiguous; pointers 16-byte aligned.
@@ -406,8 +407,8 @@ int tf_prompt_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
  * Packed tokens [T, hkv, D] (strides of tokens and heads in elements,
  * multiples of 8) of S sequences with device offsets cu[S + 1]: token i of
  * sequence s is at position start[s] + i (start may be null: 0) of cache row
- * slots[s] (may be null: s). Tokens outside [0, t_max) x [0, B) are not
- * written, and read as zeros.
+ * slots[s] (may be null: s). Tokens outside [0, t_max) x [0, B), before cu[0]
+ * or from cu[S] on are not written, and read as zeros.
  * tf_kv4_write quantises keys and values into the cache; tf_rope_kv4_write
  * first rotates the q and k heads of projection rows [T, (hq + 2 hkv) * D]
  * in place (tables [>= t_max, D], rounding as tf_rope_kv_append); tf_kv4_read

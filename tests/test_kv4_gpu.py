@@ -400,3 +400,27 @@ def test_one_token_or_one_head_of_odd_strides(dtype):
     kernels.kv4_write(k1, v1, want, cu([5]))
     kernels.kv4_write(many(k1), many(v1), got, cu([5]))
     assert all(same_bits(x, y) for x, y in zip(got, want))
+
+
+def test_tokens_in_no_sequence():
+    """Rows before cu[0] and from cu[S] on (padding to a fixed size) belong to nobody: not written, not
+    rotated, read as zeros."""
+    h, hq, d, dtype = 2, 4, 64, torch.bfloat16
+    offs, start = i32(2, 5, 9), i32(4, 10)
+    k, v = tokens(12, h, d, dtype)
+    want, got = (KV4Cache.empty(2, h, 32, d, 64, dtype) for _ in range(2))
+    kernels.kv4_write(k[2:9], v[2:9], want, cu([3, 4]), start)
+    kernels.kv4_write(k, v, got, offs, start)
+    assert all(same_bits(a, b) for a, b in zip(got, want))
+    for x, y in zip(kernels.kv4_read(random_cache(2, h, 32, d, 64, dtype), offs, 12, start),
+                    kernels.kv4_read(random_cache(2, h, 32, d, 64, dtype), cu([3, 4]), 7, start)):
+        assert torch.equal(x[2:9], y) and (x[:2] == 0).all() and (x[9:] == 0).all()
+    gen = torch.Generator("cuda").manual_seed(3)
+    rows = torch.randn(12, (hq + 2 * h) * d, device="cuda", generator=gen).to(dtype)
+    ang = torch.rand(32, d // 2, device="cuda", generator=gen) * 6
+    cos, sin = (torch.cat([f(ang), f(ang)], -1).to(dtype) for f in (torch.cos, torch.sin))
+    some, every = rows[2:9].clone(), rows.clone()
+    kernels.rope_kv4_write(some, hq, cos, sin, want, cu([3, 4]), start)
+    kernels.rope_kv4_write(every, hq, cos, sin, got, offs, start)
+    assert all(same_bits(a, b) for a, b in zip(got, want))
+    assert torch.equal(every, torch.cat([rows[:2], some, rows[9:]]))

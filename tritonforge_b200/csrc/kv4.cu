@@ -23,12 +23,14 @@ struct Kv4Rows {
 };
 
 // Cache row (in rows of D channels) of packed token t's kv head 0, or -1 outside
-// the cache; the other heads' follow t_max rows apart. `pos` is its position.
+// the cache or in no sequence (before cu[0], from cu[S] on); the other heads'
+// follow t_max rows apart. `pos` is its position.
 __device__ __forceinline__ int64_t cache_row(const Kv4Rows& a, int64_t t, int64_t& pos) {
   const int s = packed_sequence(a.cu, a.S, t);
-  pos = t - a.cu[s] + (a.start ? a.start[s] : 0);
+  const int64_t in = t - a.cu[s];
+  pos = in + (a.start ? a.start[s] : 0);
   const int64_t b = a.slots ? a.slots[s] : s;
-  if (pos < 0 || pos >= a.t_max || b < 0 || b >= a.B) return -1;
+  if (in < 0 || t >= a.cu[s + 1] || pos < 0 || pos >= a.t_max || b < 0 || b >= a.B) return -1;
   return b * a.hkv * a.t_max + pos;
 }
 

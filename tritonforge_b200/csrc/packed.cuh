@@ -1,13 +1,14 @@
 // Packed sequences: `S` sequences laid end to end in one token axis, offsets
-// cu[0..S] (device int32, cu[0] = 0, non-decreasing, cu[S] = the token count).
+// cu[0..S] (device int32, non-decreasing). Tokens before cu[0] or from cu[S] on
+// are in no sequence.
 #pragma once
 
 #include "common.cuh"
 
 namespace tf {
 
-// The sequence that token t belongs to: the last s with cu[s] <= t (empty
-// sequences own no token), in [0, S).
+// The sequence that token t belongs to, if it is in one: the last s with cu[s] <= t
+// (empty sequences own no token), in [0, S).
 __device__ __forceinline__ int packed_sequence(const int* __restrict__ cu, int S, int64_t t) {
   int lo = 0, hi = S;  // cu[lo] <= t < cu[hi]
   while (hi - lo > 1) {

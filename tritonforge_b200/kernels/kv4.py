@@ -107,7 +107,8 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, cache: KV4Cache, cu_seqlens: tor
     """Quantise packed keys and values [T, Hkv, D] into the cache: token i of
     sequence s (cu_seqlens int32 [S + 1] on the device) goes to position
     start[s] + i (start defaults to 0) of cache row slots[s] (defaults to s).
-    Tokens whose position or row lies outside the cache are left out."""
+    Tokens whose position or row lies outside the cache are left out, as are
+    rows that belong to no sequence (from cu_seqlens[S] on: padding)."""
     b, h, d, g, t_max, dt = cache.layout()
     S = _offsets(cu_seqlens)
     dtype = cache.k_params.dtype
@@ -128,7 +129,7 @@ def rope_kv4_write(qkv: torch.Tensor, q_heads: int, cos: torch.Tensor, sin: torc
     """Rotate the q and k heads of packed projection rows qkv [T, (Hq + 2 Hkv) D]
     in place (rotary tables cos/sin [>= t_max of the positions, D], transformers'
     roundings) and quantise the rotated keys and the values into the cache, as
-    kv4_write places them. Tokens outside the cache are neither rotated nor written."""
+    kv4_write places them. What kv4_write leaves out is neither rotated nor written."""
     b, h, d, g, t_max, dt = cache.layout()
     S = _offsets(cu_seqlens)
     ld = _rope_rows(qkv, q_heads, cos, sin, cache, h, d, t_max)
@@ -144,8 +145,8 @@ def kv4_read(cache: KV4Cache, cu_seqlens: torch.Tensor, total: int, start: torch
              slots: torch.Tensor | None = None, *,
              out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(k, v) [total, Hkv, D] in the cache's dtype: the values held at the
-    positions where kv4_write with the same cu_seqlens (cu_seqlens[S] = total),
-    start and slots would place packed tokens; zeros outside the cache."""
+    positions where kv4_write with the same cu_seqlens, start and slots would
+    place packed tokens; zeros for what it would leave out."""
     b, h, d, g, t_max, dt = cache.layout()
     S = _offsets(cu_seqlens)
     dev = _lib.require_cuda(*cache, cu_seqlens, start, slots)

@@ -54,8 +54,9 @@ def prompt_attention(
     S + 1 offsets; cu_seqlens_k defaults to cu_seqlens_q). With more keys than
     queries the queries are the sequence's last positions (a chunk of a prompt
     over what came before it). Causal queries see keys up to their own
-    position; a query that sees none gives zeros. `scale` is positive and
-    defaults to D**-0.5.
+    position; a query that sees none gives zeros. Rows of q in no sequence (from
+    cu_seqlens_q[S] on) are not computed: theirs of the output hold anything.
+    `out` must not overlap the inputs. `scale` is positive and defaults to D**-0.5.
     The lengths stay on the device: nothing here waits for the GPU.
     """
     shape, k_shape = q.shape, k.shape
