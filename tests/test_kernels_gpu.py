@@ -366,3 +366,19 @@ def test_qlinear_swiglu(m, i, k, dtype):
     up = oracle_linear(x, pu, su, zu, None)
     assert_swiglu_close(out, gate, up, dtype, f"qlinear_swiglu {m}x{i}x{k}")
     assert int(ws[:4].view(torch.int32).item()) == 0
+
+
+def test_outgrown_workspaces_stay():
+    """A buffer that a captured graph may still use is not given back when a larger
+    one takes its place, and the error word in it is still read."""
+    ws = _lib._Workspaces()
+    dev = torch.device("cuda", 0)
+    small = ws.get(dev, 1 << 20)
+    at, n = small.data_ptr(), small.numel()
+    small[:4].view(torch.int32).fill_(4)
+    del small
+    large = ws.get(dev, 8 << 20)
+    assert large.numel() >= 8 << 20 and ws.get(dev, 1 << 20) is large
+    others = [torch.empty(n, dtype=torch.uint8, device=dev) for _ in range(64)]
+    assert all(not at <= x.data_ptr() < at + n for x in others)
+    assert ws.errors(dev) == 4 and ws.errors(dev, clear=True) == 4 and ws.errors(dev) == 0

@@ -190,11 +190,15 @@ class _Workspaces:
 
     A buffer is zeroed only when it is (re)allocated. Reallocation happens
     outside any CUDA-graph capture: callers that capture size it first with
-    ``reserve`` (or run the captured work once on the capture stream).
+    ``reserve`` (or run the captured work once on the capture stream). A buffer
+    that has become too small is kept, for the graphs that were captured with it
+    (sizes at least double, so all of a stream's old ones together are smaller
+    than its present one) and for the error word in it.
     """
 
     def __init__(self) -> None:
         self._bufs: dict[tuple[int, int], torch.Tensor] = {}
+        self._outgrown: list[tuple[int, torch.Tensor]] = []
 
     def get(self, device: torch.device, nbytes: int) -> torch.Tensor:
         idx = device.index if device.index is not None else torch.cuda.current_device()
@@ -202,7 +206,9 @@ class _Workspaces:
         buf = self._bufs.get(key)
         if buf is None or buf.numel() < nbytes:
             size = max(nbytes, 1 << 20, 0 if buf is None else 2 * buf.numel())
-            buf = torch.zeros(size, dtype=torch.uint8, device=torch.device("cuda", idx))
+            old, buf = buf, torch.zeros(size, dtype=torch.uint8, device=torch.device("cuda", idx))
+            if old is not None:
+                self._outgrown.append((idx, old))
             self._bufs[key] = buf
         return buf
 
@@ -214,7 +220,7 @@ class _Workspaces:
         all devices): 0 when every kernel that used them completed its bounded
         waits. Synchronises the devices involved; `clear` zeroes the words."""
         bits = 0
-        for (idx, _), buf in list(self._bufs.items()):
+        for idx, buf in self._outgrown + [(idx, buf) for (idx, _), buf in self._bufs.items()]:
             if device is not None and device.index is not None and idx != device.index:
                 continue
             torch.cuda.synchronize(idx)
