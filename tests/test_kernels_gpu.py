@@ -382,3 +382,15 @@ def test_outgrown_workspaces_stay():
     others = [torch.empty(n, dtype=torch.uint8, device=dev) for _ in range(64)]
     assert all(not at <= x.data_ptr() < at + n for x in others)
     assert ws.errors(dev) == 4 and ws.errors(dev, clear=True) == 4 and ws.errors(dev) == 0
+
+
+@pytest.mark.parametrize("family", ["workspaces", "kv4_workspaces", "prompt_workspaces"])
+def test_device_errors(family):
+    """A bit in any workspace's error word shows in kernels.device_errors, and is cleared there."""
+    dev = torch.device("cuda", 0)
+    assert kernels.device_errors() == kernels.device_errors(dev) == 0
+    getattr(_lib, family).get(dev, 1 << 20)[:4].view(torch.int32).fill_(2)
+    assert kernels.device_errors() == kernels.device_errors(dev) == 2
+    assert kernels.device_errors(torch.device("cuda", 1)) == 0
+    assert kernels.device_errors(dev, clear=True) == 2
+    assert kernels.device_errors() == 0

@@ -235,3 +235,14 @@ workspaces = _Workspaces()
 # the 4-bit cache's and the prompts' attention leave partial results where the others keep counters: buffers of their own
 kv4_workspaces = _Workspaces()
 prompt_workspaces = _Workspaces()
+
+
+def device_errors(device: torch.device | None = None, clear: bool = False) -> int:
+    """Error bits that this process's kernels left on `device` (or on all): a
+    wait inside a kernel gave up after 1 s, and the output of that launch, which
+    reported success, is not to be trusted. 0: every launch ran to its end.
+    Waits for the devices involved; `clear` zeroes the words."""
+    bits = 0
+    for ws in (workspaces, kv4_workspaces, prompt_workspaces):
+        bits |= ws.errors(device, clear)
+    return bits

@@ -450,14 +450,11 @@ class QwenDecoder:
         return int(self._ar_err.item()) if self.fused_allreduce else 0
 
     def device_errors(self) -> int:
-        """Error bits the decode kernels left on this device: the fused
-        all-reduce's word and the int4 kernels' workspace words (a bounded
+        """Error bits the kernels left on this device: the fused all-reduce's
+        word and the workspaces' words (kernels.device_errors: a bounded
         wait that gave up after 1 s). 0 means every launch ran to the end;
         anything else means the outputs of some step are not to be trusted."""
-        errs = self.allreduce_errors() | _lib.workspaces.errors(self.dev)
-        if self.kv4 is not None:
-            errs |= _lib.kv4_workspaces.errors(self.dev) | _lib.prompt_workspaces.errors(self.dev)
-        return errs
+        return self.allreduce_errors() | _lib.device_errors(self.dev)
 
     # ------------------------------------------------------------------ step
     def _lin(self, x: torch.Tensor, ql, out: torch.Tensor) -> torch.Tensor:
