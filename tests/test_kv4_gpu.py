@@ -424,3 +424,35 @@ def test_tokens_in_no_sequence():
     kernels.rope_kv4_write(every, hq, cos, sin, got, offs, start)
     assert all(same_bits(a, b) for a, b in zip(got, want))
     assert torch.equal(every, torch.cat([rows[:2], some, rows[9:]]))
+
+
+def check_finite(got, q, cache, lens):
+    """check_decode, where a NaN (its difference is not above a tolerance either) fails too."""
+    assert torch.isfinite(got.float()).all(), f"{int((~torch.isfinite(got.float())).sum())} of {got.numel()} not finite"
+    check_decode(got, q, cache, lens)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d,g", [(64, 64), (128, 64), (128, 128)])
+@pytest.mark.parametrize("qs,vs", [(1e-4, 1.0), (30.0, 1e-3), (1.0, 200.0), (3.0, 1e-5), (2e3, 3e3), (0.0, 1.0), (1.0, 0.0)])
+def test_decode_magnitudes_stay_finite(qs, vs, d, g, dtype):
+    """Queries and values far from 1, all zero among them: finite results of the same precision."""
+    lens = [700, 33]
+    cache = random_cache(2, 4, 704, d, g, dtype, v_size=vs)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q = (torch.randn(2, 28, d, device="cuda", generator=gen) * qs).to(dtype)
+    check_finite(kernels.kv4_decode_attention(q, cache, i32(*lens)), q, cache, lens)
+
+
+@pytest.mark.parametrize("up", [True, False])
+def test_decode_mixed_value_scales_stay_finite(up):
+    """Value scales over eight orders of magnitude along the context, growing and shrinking."""
+    n, dtype = 900, torch.bfloat16
+    cache = KV4Cache.empty(1, 2, 912, 128, 64, dtype)
+    gen = torch.Generator(device="cuda").manual_seed(10)
+    ramp = 10.0 ** torch.linspace(-4, 4, n, device="cuda")
+    k = torch.randn(n, 2, 128, device="cuda", generator=gen)
+    vals = torch.randn(n, 2, 128, device="cuda", generator=gen) * (ramp if up else ramp.flip(0))[:, None, None]
+    kernels.kv4_write(k.to(dtype), vals.to(dtype), cache, cu([n]))
+    q = torch.randn(1, 14, 128, device="cuda", generator=gen).to(dtype)
+    check_finite(kernels.kv4_decode_attention(q, cache, i32(n)), q, cache, [n])
