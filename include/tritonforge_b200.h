@@ -412,7 +412,7 @@ int tf_prompt_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
  * tf_kv4_write quantises keys and values into the cache; tf_rope_kv4_write
  * first rotates the q and k heads of projection rows [T, (hq + 2 hkv) * D]
  * in place (tables [>= t_max, D], rounding as tf_rope_kv_append); tf_kv4_read
- * returns the values. */
+ * returns the values (its rows must not overlap: strides at least D). */
 int tf_kv4_write(const void* k, int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
                  int64_t v_stride_h, uint8_t* k_codes, void* k_params, uint8_t* v_codes, void* v_params,
                  const int* cu, const int* start, const int* slots, int32_t S, int64_t T, int64_t B, int32_t hkv,

@@ -83,6 +83,17 @@ def test_kv4_refusals():
     assert attend(B=0) == _lib.OK
 
 
+def test_kv4_read_refuses_rows_that_overlap():
+    """Rows written over each other (an expanded output): no order among them."""
+    def read(ks, vs, T=4, h=2):
+        return _lib.load().tf_kv4_read(P, P, P, P, P, *ks, P, *vs, P, None, None, 1, T, 1, h, 128, 64, 64, _lib.F16, None)
+
+    good = (256, 128)
+    for bad in ((0, 128), (256, 0), (64, 128), (256, 64)):
+        assert read(bad, good) == read(good, bad) == _lib.ERR_BAD_SHAPE
+    assert read((0, 0), good) == read((0, 128), good, h=1) == read((256, 0), good, T=1) == _lib.ERR_BAD_SHAPE
+
+
 def test_logprobs_refusals():
     def call(x=P, ld=100, t=P, M=2, V=100, top=3, dtype=_lib.F32, out=P, ids=P):
         return _lib.load().tf_token_logprobs(x, ld, t, M, V, top, dtype, out, out, out, ids, None)

@@ -240,6 +240,9 @@ extern "C" int tf_kv4_read(const uint8_t* k_codes, const void* k_params, const u
   if (rc != TF_OK || T == 0) return rc;
   rc = check_rows("kv4_read", k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, T, hkv);
   if (rc != TF_OK) return rc;
+  if ((T > 1 && (k_stride_t < head_dim || v_stride_t < head_dim)) ||
+      (hkv > 1 && (k_stride_h < head_dim || v_stride_h < head_dim)))
+    return fail(TF_ERR_BAD_SHAPE, "kv4_read: output rows overlap");
   const Kv4Rows a{c, cu, start, slots, T, B, t_max, S, hkv};
   return kv4_dispatch(dtype, head_dim, group, [&](auto type, auto d, auto g) {
     using E = std::remove_pointer_t<decltype(type)>;
