@@ -456,3 +456,24 @@ def test_decode_mixed_value_scales_stay_finite(up):
     kernels.kv4_write(k.to(dtype), vals.to(dtype), cache, cu([n]))
     q = torch.randn(1, 14, 128, device="cuda", generator=gen).to(dtype)
     check_finite(kernels.kv4_decode_attention(q, cache, i32(n)), q, cache, [n])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d,g", [(64, 64), (128, 64), (128, 128)])
+@pytest.mark.parametrize("n", [8, 900])
+def test_small_weights_beside_a_large_one(n, d, g, dtype):
+    """One position takes nearly all of the weight, and all but two values of a group are zero there (their
+    codes the zero point); the others weigh e^-11.5 to e^-13.5 each, with the largest code. Their sum must
+    not drown in the products of the first with its codes, which the zero points take away again."""
+    h = 16
+    gen = torch.Generator(device="cuda").manual_seed(d + g)
+    q = torch.randn(1, h, d, device="cuda", generator=gen).to(dtype)
+    gap = torch.linspace(11.5, 13.5, h, device="cuda")[:, None]
+    k = torch.zeros(n, h, d, device="cuda")
+    k[5] = q[0].float() * gap * d ** 0.5 / q[0].float().pow(2).sum(-1, keepdim=True)
+    v = torch.full((n, h, d), 63.0, device="cuda")  # groups of scale 126 / 15, zero point 8
+    v[5] = 0
+    v[:, :, ::g], v[:, :, 1::g] = -63, 63
+    cache = KV4Cache.empty(1, h, n, d, g, dtype)
+    kernels.kv4_write(k.to(dtype), v.to(dtype), cache, cu([n]))
+    check_finite(kernels.kv4_decode_attention(q, cache, i32(n)), q, cache, [n])

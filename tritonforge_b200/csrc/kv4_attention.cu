@@ -4,13 +4,22 @@
 // with k_t, v_t the values the codes stand for, (code - zero) * scale:
 //   q . k_t = s_t (sum_d q_d c_td - z_t sum_d q_d)   per group of channels,
 //   out     = sum_t p_t s_t (c_td - z_t).
-// Scores, softmax and sums are in fp32, the output is rounded once; a sequence
+// Softmax and accumulators are in fp32, the output is rounded once; a sequence
 // without positions gives zeros. The bound is the bytes of the cached rows.
 //
 // Products: mma.sync on the codes themselves. A 4-bit code under the mask
 // 0x000f000f is a subnormal fp16 number, code 2^-24, under 0x00f000f0 16 times
 // that: no conversion at all, the powers of two go into the other operand or
-// into the result. Per 16 positions a warp takes S^T = K Q^T (rows: positions,
+// into the result. The tensor cores line addends up by their exponents, a
+// subnormal's being -14 whatever its leading zeros, and drop what lies 2^-24 below
+// the largest: beside a code of 8 addends are kept to 2^-17 of it under the first
+// mask, to 2^-21 under the second. The values' sums, from which the zero points take
+// most away again, use the second for both nibbles (a shift; 32 x 4096, 64 / 8
+// heads: 37.3 -> 37.9 us; code - zero as normal numbers 48). Scores keep the first
+// for every other nibble: 2^-15 of the largest |q| a product, which does not show
+// beside the rounded weights (the second for all of them: 39.9 us, errors against
+// 64 bits equal, also with one channel of q 400 times the others).
+// Per 16 positions a warp takes S^T = K Q^T (rows: positions,
 // columns: up to 8 query heads of the kv head) and O^T += V^T P^T; a row of the
 // cache is read as it lies, its channels in whatever order the nibbles come
 // (the same for q). tcgen05 would want the codes as 16-bit operands in shared
@@ -30,7 +39,7 @@
 // order: results do not depend on timing. One warp streams the share through a
 // ring in shared memory (bulk copies), four compute, 32 positions of a unit each.
 //
-// Batch 32 x 4096 positions: 37.3 us with 64 / 8 heads of 128, 59% of the copy
+// Batch 32 x 4096 positions: 37.9 us with 64 / 8 heads of 128, 59% of the copy
 // bandwidth, 25.3 with 28 / 4, 13.7 with 14 / 2 heads of 64. Two or three warps a
 // scheduler issue in 44% of the cycles, each waiting for its own chain of products,
 // exponentials and shuffles, and about 8 us go to the start and the joins: that is
@@ -632,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D>) kv4_attn_kernel(const
               const uint32_t sel = 0x4400u + 0x1111u * (j & 3);  // byte j of both, in bits 0-7 and 16-23
               const uint32_t lo = __byte_perm(vw[0][j / 4], vw[1][j / 4], sel);
               const uint32_t hi = __byte_perm(vw[2][j / 4], vw[3][j / 4], sel);
-              const uint32_t f[4] = {lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u};
+              const uint32_t f[4] = {(lo << 4) & 0x00f000f0u, lo & 0x00f000f0u, (hi << 4) & 0x00f000f0u, hi & 0x00f000f0u};
               mma16816(acc[g * VB + j], f, pb[u][g][0], pb[u][g][1]);
             }
           }
@@ -659,11 +668,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<D>) kv4_attn_kernel(const
       for (int j = 0; j < VB; ++j) {
         const float* v = acc[g * VB + j];
         const int d = g * GS + r * (GS / 8) + 2 * j;
-        const float two24 = 16777216.f;
+        const float two20 = 1048576.f;
         *reinterpret_cast<float2*>(&sm.o[warp][2 * c][d]) =
-            make_float2((v[0] * two24 - za[g][0]) * back, (v[2] * (two24 / 16.f) - za[g][0]) * back);
+            make_float2((v[0] * two20 - za[g][0]) * back, (v[2] * two20 - za[g][0]) * back);
         *reinterpret_cast<float2*>(&sm.o[warp][2 * c + 1][d]) =
-            make_float2((v[1] * two24 - za[g][1]) * back, (v[3] * (two24 / 16.f) - za[g][1]) * back);
+            make_float2((v[1] * two20 - za[g][1]) * back, (v[3] * two20 - za[g][1]) * back);
       }
     if (r == 0) {
       sm.m[warp][2 * c] = m0;
