@@ -3,9 +3,10 @@
 // lanes, each holding channels [8i, 8i + 8) and [D/2 + 8i, D/2 + 8i + 8): two
 // 16-byte loads, the group minima and maxima by shuffles, and the two channels
 // of a rotary pair always in one lane.
-// 20011 tokens of 8 heads of 128, bf16, groups of 128: written in 27.0 us, read in
-// 22.9, 59% and 69% of the copy bandwidth (104 MB each; with 14 / 2 heads of 64 or
-// few tokens it is the launch). Instruction issue bounds both: about 15
+// 20011 tokens of 8 heads of 128, bf16, groups of 128: written in 27.4 us, read in
+// 22.7, 58% and 70% of the copy bandwidth (104 MB each; with 14 / 2 heads of 64 or
+// few tokens it is the launch); 64 query and 8 key heads rotated and keys and values
+// written in 196 us, 62% (801 MB). Instruction issue bounds both: about 15
 // instructions a channel and lane to write, and loads of 4 bytes a lane to read.
 #include "kv4.cuh"
 #include "packed.cuh"

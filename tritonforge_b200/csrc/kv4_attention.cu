@@ -39,12 +39,13 @@
 // order: results do not depend on timing. One warp streams the share through a
 // ring in shared memory (bulk copies), four compute, 32 positions of a unit each.
 //
-// Batch 32 x 4096 positions: 37.9 us with 64 / 8 heads of 128, 59% of the copy
-// bandwidth, 25.3 with 28 / 4, 13.7 with 14 / 2 heads of 64. Two or three warps a
-// scheduler issue in 44% of the cycles, each waiting for its own chain of products,
-// exponentials and shuffles, and about 8 us go to the start and the joins: that is
-// all of it for short batches (300 positions: 4.8 us; 16 sequences of 1125 on
-// average, 28 / 4 heads: 13.7).
+// In a CUDA graph, 32 x 4096 positions: 38.1 us with 64 / 8 heads of 128, 58% of the
+// copy bandwidth, 25.9 with 28 / 4, 14.0 with 14 / 2 heads of 64; rotating and
+// appending the new token too (the fused form) 44.3, 29.9 and 16.8. Two or three
+// warps a scheduler issue in 47% of the cycles, each waiting for its own chain of
+// products, exponentials and shuffles, and about 8 us go to the start and the joins:
+// that is all of it for short batches (300 positions: 5.0 us, fused 6.6; 16 sequences
+// of 1125 on average, 28 / 4 heads: 14.0, fused 17.8).
 #include "kv4.cuh"
 
 namespace tf {

@@ -18,13 +18,17 @@
 // Alternatives: a logit is a candidate when it reaches a bound that n logits of
 // the CTA's part reach for certain: with k = ceil(n / warps), the least over the
 // warps of the k-th largest of its 32 lane maxima. The bound rises as the pass
-// goes on, so of V random logits only some hundreds are looked at again.
+// goes on, so of V random logits only some hundreds are looked at again. It cannot
+// rise while a warp has seen fewer than k logits above -inf: where a mask leaves only
+// a few ids, or one range of them, every logit is looked at (32 rows of 152064 with 10
+// ids or 1000 in a row allowed, 20 alternatives: 56 and 60 us, against 18).
 // Candidates wait in a buffer per warp, cut back to its n largest when full; at
 // the end the CTA ranks the survivors by counting.
-// 2048 rows of 152064 bf16 logits: 109 us without alternatives, 125 with 8 (87% and
-// 76% of the copy bandwidth; fp32 195); instruction issue bounds it. 32 rows: 8 us
-// without, 13 with 5, 18 with 20: a chain of latencies (the copies, two steps of
-// 32 logits a thread, the candidates, the joins, one meeting of the cluster).
+// In a CUDA graph, 2048 rows of 152064 bf16 logits: 105 us without alternatives, 125
+// with 8 (91% and 76% of the copy bandwidth; in a call, inputs alternating, 137);
+// 1024 rows in fp32 with 8 111 (85%); instruction issue bounds it. 32 rows: 8 us
+// without, 13 with 5, 18 with 20: a chain of latencies (the copies, two steps of 32
+// logits a thread, the candidates, the joins, one meeting of the cluster).
 #include <cooperative_groups.h>
 
 #include "common.cuh"

@@ -39,9 +39,10 @@
 // rows that do not see them come out as if they were not there, and in the others
 // the channel becomes what the sum is, an infinity or NaN.
 //
-// 8192 tokens of 64 / 8 heads of 128: 845 us, 79% of the measured tensor rate (980
-// in a run of seconds, under the power cap); 701 queries over 9702 keys 94 us; 4099
-// tokens in 11 prompts of 28 / 4 heads 38; 37 tokens of 14 / 2 heads of 64 9. A pair of tiles takes 3300 to 3500 cycles a
+// In a CUDA graph, 8192 tokens of 64 / 8 heads of 128: 850 us, 79% of the measured
+// tensor rate (980 in a run of seconds, under the power cap); 701 queries over 9702
+// keys 93 us; 4099 tokens in 11 prompts of 28 / 4 heads 37; 6000 tokens of 14 / 2
+// heads of 64 114; 37 tokens of them 8. A pair of tiles takes 3300 to 3500 cycles a
 // block for 2048 of products: a tile's own chain (scores to registers and maximum
 // 720, powers and P 1500, the last quarter's product and the next S 1000) is what
 // is left, TMEM being full; a pair costs 2000 to 4000 cycles more for its first
